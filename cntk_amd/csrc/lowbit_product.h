@@ -114,7 +114,8 @@ struct Bf16Op
     }
 };
 
-// A run of memory that the lanes of a wavefront copy from: nothing is read from its end on, whatever the offset.
+// A run of memory that the lanes of a wavefront copy from: a lane whose own offset lies at its end or beyond reads nothing and gets zeros. The offset
+// that all lanes share takes no part in that check.
 struct Span
 {
     const char* base;
@@ -125,7 +126,7 @@ __device__ __forceinline__ Span span(const char* base, uint64_t bytes)
     return {base, bytes < 0xffffffffu ? (uint32_t) bytes : 0xffffffffu};
 }
 // One lane's copy of 16 (4) bytes straight to LDS: `lane_at` + `at` is the place in the span, `to` the wavefront's place in LDS, where the
-// lanes follow one another.
+// lanes follow one another. Whether a lane reads is a matter of `lane_at` alone: with any `at` that is used, a lane below the span's end stays below it.
 template <int BYTES>
 __device__ __forceinline__ void copy_to_lds(const Span& from, uint32_t lane_at, uint32_t at, char* to)
 {
@@ -318,15 +319,17 @@ struct TileKernel
 
     __device__ __forceinline__ uint32_t blocks() const { return p_blocks * q_blocks; }
 
-    // the tiles of t from `first` on, and the scale group that is the wavefront's, `group` of t
+    // The tiles of t from `first` on, and the scale group that is the wavefront's, `group` of t, or the last one.
+    // A lane's offset is a whole number of rows of tiles and a place in a tile, the shared one is less than a row.
     static __device__ __forceinline__ Span tiles_from(const Tiles& t, uint32_t first)
     {
         const uint64_t row_bytes = (uint64_t) t.k_tiles * kTileBytes;
         return span(t.tiles + first * row_bytes, first < t.row_tiles ? (t.row_tiles - first) * row_bytes : 0);
     }
+    // All rows from column 16 * first on. (Whole stages end beyond the last row: the stage's offset is added to the lanes' own, which are checked.)
     static __device__ __forceinline__ Span tiles_from(const Columns& t, uint32_t first)
     {
-        return first * 16 < t.cols ? span(t.base + first * 32, (uint64_t) (t.rows - 1) * t.pitch + (t.cols - first * 16) * 2) : span(t.base, 0);
+        return span(t.base + first * 32, (uint64_t) (t.rows - 1) * t.pitch + (t.cols - first * 16) * 2);
     }
     // tile t of a row of a stage lies where tile t ^ exchange(row) would
     static __device__ __forceinline__ uint32_t exchange(uint32_t row)
@@ -341,13 +344,14 @@ struct TileKernel
     static __device__ __forceinline__ Span scales_of(const Tiles& t, uint32_t group)
     {
         const uint64_t group_bytes = (uint64_t) t.k_tiles * kScaleGroupBytes;
-        return span(t.scales + group * group_bytes, group * 4 < t.row_tiles ? group_bytes : 0);
+        return span(t.scales + min(group, (t.row_tiles - 1) / 4) * group_bytes, group_bytes);
     }
     __device__ __forceinline__ void aim(uint32_t block, Spans& s) const
     {
         uint32_t bp, bq;
         block_of(block, p_blocks, q_blocks, bp, bq);
-        s.q = tiles_from(q, bq * kQTiles + wave * kQCopies);
+        // (beyond the last tile it is that one, whose results are not written: an empty span would leave it to the shared offset what is read)
+        s.q = tiles_from(q, min(bq * kQTiles + wave * kQCopies, q.row_tiles - 1));
         s.p = tiles_from(p, bp * kPTiles);
         if constexpr (Op::kScaled)
         {
@@ -370,7 +374,7 @@ struct TileKernel
             copy_to_lds<16>(spans.q, q_lane_at[i], q_at, to + (wave * kQCopies + i) * kTileBytes);
 #pragma unroll
         for (int i = (I + 2) % TQ; i < kPCopies; i += TQ)
-            copy_to_lds<16>(spans.p, p_lane_at[i], p_at, to + (kQTiles + p_tile(i)) * kTileBytes);
+            copy_to_lds<16>(spans.p, p_lane_at[i] + (kTurned ? p_at : 0), kTurned ? 0 : p_at, to + (kQTiles + p_tile(i)) * kTileBytes);
         if constexpr (Op::kScaled && I == 1)
             copy_to_lds<4>(spans.q_scales, lane * 4, scale_at, to + kTileLds + min(wave, (uint32_t) kQGroups - 1) * kScaleGroupBytes);
         if constexpr (Op::kScaled && I == 3)

@@ -434,6 +434,23 @@ def test_weight_gradients_from_gradients_as_they_lie(m, k, n):
     assert bad[n - 1].all() and int(bad.sum()) == k + int(bad[9].sum())
 
 
+@pytest.mark.parametrize("m", [1, 31, 64, 70, 95, 257])
+@pytest.mark.parametrize("k,n", [(1000, 1288), (264, 4104), (700, 2056), (136, 9304), (2050, 5000)])
+def test_weight_gradients_do_not_see_the_rows_below(m, k, n):
+    """The gradient's rows are the first ones of a taller matrix, whose other rows hold NaN and infinities: whole stages of the product end
+    beyond the last row, and what lies there takes no part."""
+    kept = lowbit.save8(make(1, m, k, torch.bfloat16))
+    near = make(2, m, n, torch.bfloat16)
+    dw, db = lowbit.weight_gradient(near, kept, bias=True)
+    assert torch.isfinite(dw).all() and torch.isfinite(db).all()
+    for beside in (0, 24):
+        tall = torch.full((m + 160, n + beside), float("nan"), dtype=torch.bfloat16, device="cuda")
+        tall[m + 1::2] = float("inf")
+        tall[:m, :n] = near
+        got, got_db = lowbit.weight_gradient(tall[:m, :n], kept, bias=True)
+        assert torch.equal(got, dw) and torch.equal(got_db, db)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("m,k,n", [(1300, 2, 100001), (1300, 100001, 2), (1500, 16, 20000), (1025, 33, 9303), (1030, 64, 20001), (700, 30001, 60), (1100, 700, 900),
                                    (1024, 900, 900), (2000, 500, 500), (1200, 2000, 1000), (96, 1900, 1101), (300, 70000, 1), (65, 1, 70000)])
