@@ -413,7 +413,9 @@ PyObject* weight_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     packed(saved);
     same_device(dy, saved);
     const int64_t k = integer(args[2]);
-    const bool bias = integer(args[3]) != 0;
+    const bool bias = integer(args[3]) != 0, accumulate = integer(args[6]) != 0;
+    if (accumulate && (args[4] == Py_None || (bias && args[5] == Py_None)))
+        refuse("accumulate needs every result's tensor to add to");
     const Rows r = rows_of(dy, true);
     const at::Tensor dw = result(args[4], {r.cols, k}, at::kFloat, dy);
     at::Tensor db, work;
@@ -424,7 +426,7 @@ PyObject* weight_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         work = bytes(need, dy);
     check(cntkq_weight_gradient_async(handle(dy.get_device()), r.data, code, r.row_stride, r.rows, r.cols, saved.data_ptr(), saved.numel(), k,
                                       static_cast<float*>(dw.data_ptr()), row_stride(dw), bias ? static_cast<float*>(db.data_ptr()) : nullptr,
-                                      (int) integer(args[6]), need != 0 ? work.data_ptr() : nullptr, need));
+                                      accumulate, need != 0 ? work.data_ptr() : nullptr, need));
     return bias ? pair(dw, db) : THPVariable_Wrap(dw);
     END_HANDLE_TH_ERRORS
 }

@@ -190,13 +190,12 @@ def activation_backward(dy, kept):
 
 def weight_gradient(dy, kept, bias=False, out=None, accumulate=False):
     """dw = dy' x8 (n x k, float32) from the layer's input as kept (save8, mx4_linear(save=True)); with bias=True (dw, db), db the column
-    sums of dy. out: dw, or the pair (dw, db), to write into; accumulate: added to what it holds."""
+    sums of dy. out: dw, or the pair (dw, db), to write into, either of them None for a new tensor; accumulate: added to what they hold, both
+    given then."""
     if kept.kind is not None:
         raise QuantizerLogicError("what was kept belongs to an activation")
     if dy.shape[:-1] != kept.shape[:-1]:
         raise QuantizerLogicError("dy has other rows (%s) than the kept input (%s)" % (tuple(dy.shape), tuple(kept.shape)))
-    if accumulate and out is None:
-        raise QuantizerLogicError("accumulate needs the tensors to add to")
     dw, db = (None, None) if out is None else (out if bias else (out, None))
     return _ops.weight_gradient(dy, kept.buffer, kept.shape[-1], bias, dw, db, accumulate)
 

@@ -627,6 +627,28 @@ def test_refusals():
             call()
 
 
+def test_adding_needs_every_result():
+    """A result that is to be added to and is not given would be added to memory that nobody has written."""
+    x, dy = make(1, 20, 40, torch.bfloat16), make(2, 20, 30, torch.bfloat16)
+    kept = lowbit.save8(x)
+    dw, db = torch.zeros(30, 40, device="cuda"), torch.zeros(30, device="cuda")
+    for given in (None, (dw, None), (None, db), (None, None)):
+        with pytest.raises(QuantizerLogicError):
+            lowbit.weight_gradient(dy, kept, bias=True, out=given, accumulate=True)
+    with pytest.raises(QuantizerLogicError):
+        lowbit.weight_gradient(dy, kept, accumulate=True)
+    assert not dw.any() and not db.any()
+    want, want_db = lowbit.weight_gradient(dy, kept, bias=True)
+    # one of two given, to write into
+    for given in ((dw, None), (None, db)):
+        got, got_db = lowbit.weight_gradient(dy, kept, bias=True, out=given)
+        assert torch.equal(got, want) and torch.equal(got_db, want_db)
+    lowbit.weight_gradient(dy, kept, bias=True, out=(dw, db), accumulate=True)
+    assert torch.equal(dw, 2.0 * want) and torch.equal(db, 2.0 * want_db)
+    lowbit.weight_gradient(dy, kept, out=dw, accumulate=True)
+    assert torch.allclose(dw, 3.0 * want, rtol=2.0 ** -22, atol=0.0) and torch.equal(db, 2.0 * want_db)
+
+
 # ---- modules --------------------------------------------------------------------------------------
 
 
