@@ -97,21 +97,27 @@ void same_device(const at::Tensor& a, const at::Tensor& b)
 // a packed matrix's buffer
 void packed(const at::Tensor& t)
 {
-    if (t.scalar_type() != at::kByte || !t.is_cuda() || !t.is_contiguous())
+    if (t.scalar_type() != at::kByte || !t.is_cuda() || !t.is_contiguous() || t.is_neg())
         refuse("a packed matrix is a contiguous uint8 device tensor");
 }
 
 // A tensor as a matrix of its last dimension's rows: in place where its strides allow one (and, if asked for, the values of a row are
-// neighbours), a copy otherwise.
+// neighbours), a copy otherwise. (A view that stands for its memory's negative is a copy too: data_ptr() does not know of the sign.)
 struct Rows
 {
     at::Tensor kept; // the copy
     const void* data;
     int64_t rows, cols, row_stride, col_stride;
 };
-Rows rows_of(const at::Tensor& t, bool contiguous)
+Rows rows_of(const at::Tensor& given, bool contiguous)
 {
     Rows r;
+    if (given.is_neg())
+    {
+        at::NoGradGuard no_grad;
+        r.kept = given.resolve_neg();
+    }
+    const at::Tensor t = r.kept.defined() ? r.kept : given;
     if (t.dim() == 2)
     {
         r.rows = t.size(0);
@@ -154,6 +160,8 @@ at::Tensor result(PyObject* out, at::IntArrayRef sizes, at::ScalarType type, con
     const at::Tensor& t = tensor(out, "out");
     if (t.sizes() != sizes || t.scalar_type() != type || t.device() != like.device())
         refuse("out has another shape, type or device than the result");
+    if (t.is_neg())
+        refuse("out is a view that stands for its memory's negative");
     if (t.dim() == 2 ? t.size(1) > 1 && t.stride(1) != 1 : !t.is_contiguous())
         refuse("out must have contiguous rows");
     return t;
@@ -187,10 +195,10 @@ Bias bias_of(PyObject* o, int64_t n, const at::Tensor& like)
     if (t.dim() != 1 || t.size(0) != n)
         refuse("bias must have one element per row of the weights");
     same_device(like, t);
-    if (n > 1 && t.stride(0) != 1)
+    if (t.is_neg() || (n > 1 && t.stride(0) != 1))
     {
         at::NoGradGuard no_grad;
-        b.kept = t.contiguous();
+        b.kept = t.resolve_neg().contiguous();
         b.data = b.kept.data_ptr();
     }
     else

@@ -627,6 +627,49 @@ def test_refusals():
             call()
 
 
+def negated(t):
+    """A view with t's values over memory that holds their negatives."""
+    v = torch._neg_view(-t)
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_views_that_stand_for_their_negative(dtype):
+    x, w, dy = make(1, 24, 40, dtype), make(2, 30, 40, dtype), make(3, 24, 30, dtype)
+    bias = make(4, 1, 30, dtype).view(30)
+    q = lowbit.mx4_quantize(w)
+    for shape in ((24, 40), (2, 3, 4, 40)):
+        v = x.view(shape)
+        assert torch.equal(lowbit.mx4_quantize(negated(v)).buffer, lowbit.mx4_quantize(x).buffer)
+        assert torch.equal(lowbit.save8(negated(v)).buffer, lowbit.save8(x).buffer)
+        y, kept = lowbit.mx4_linear(v, q, bias, save=True)
+        y_, kept_ = lowbit.mx4_linear(negated(v), q, negated(bias), save=True)
+        assert torch.equal(y, y_) and torch.equal(kept.buffer, kept_.buffer)
+        assert torch.equal(lowbit.mx4_linear(negated(v)[:1], q, negated(bias)), lowbit.mx4_linear(v[:1], q, bias))
+        d = dy.view(shape[:-1] + (30,))
+        for a, b in zip(lowbit.weight_gradient(negated(d), kept, bias=True), lowbit.weight_gradient(d, kept, bias=True)):
+            assert torch.equal(a, b)
+        z, held = lowbit.activation_forward("silu", v, v)
+        z_, held_ = lowbit.activation_forward("silu", negated(v), negated(v))
+        assert torch.equal(z, z_) and torch.equal(held.buffer, held_.buffer) and torch.equal(held.gate, held_.gate)
+        for a, b in zip(lowbit.activation_backward(negated(v), held), lowbit.activation_backward(v, held)):
+            assert torch.equal(a, b)
+    assert torch.equal(lowbit.mx4_quantize(negated(w).t()).buffer, lowbit.mx4_quantize(w.t()).buffer)
+    assert torch.equal(lowbit.mx4_matmul(lowbit.mx4_quantize(x), q, negated(bias)), lowbit.mx4_matmul(lowbit.mx4_quantize(x), q, bias))
+    # the imaginary part of a conjugate is one
+    z = torch.complex(make(5, 24, 40, torch.float32), make(6, 24, 40, torch.float32))
+    assert z.conj().imag.is_neg()
+    assert torch.equal(lowbit.mx4_quantize(z.conj().imag).buffer, lowbit.mx4_quantize(-z.imag).buffer)
+    # nothing is written through one
+    for call in (lambda: lowbit.mx4_linear(x, q, out=torch._neg_view(torch.zeros(24, 30, dtype=dtype, device="cuda"))),
+                 lambda: lowbit.mx4_dequantize(q, torch.float32, out=torch._neg_view(torch.zeros(30, 40, device="cuda"))),
+                 lambda: lowbit.weight_gradient(dy, kept, out=torch._neg_view(torch.zeros(30, 40, device="cuda"))),
+                 lambda: lowbit.weight_gradient(dy, kept, bias=True, out=(None, torch._neg_view(torch.zeros(30, device="cuda"))))):
+        with pytest.raises(QuantizerLogicError):
+            call()
+
+
 def test_adding_needs_every_result():
     """A result that is to be added to and is not given would be added to memory that nobody has written."""
     x, dy = make(1, 20, 40, torch.bfloat16), make(2, 20, 30, torch.bfloat16)
