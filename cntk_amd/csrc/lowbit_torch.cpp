@@ -6,6 +6,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -152,6 +153,20 @@ at::Tensor bytes(size_t n, const at::Tensor& like)
 {
     return make({(int64_t) n}, at::kByte, like);
 }
+// A tensor of the caller's that is written behind autograd's back: it must not be part of a graph, and what autograd saved of it has to show that it
+// changed (`written`, once the call is on its way; `given`: the argument).
+void writable(const at::Tensor& t)
+{
+    if (at::GradMode::is_enabled() && t.requires_grad())
+        refuse("out requires grad: the low-bit functions take part in no autograd graph");
+    if (t.is_inference() && !c10::InferenceMode::is_enabled())
+        refuse("out was made in inference mode and is written outside of it");
+}
+void written(PyObject* given, const at::Tensor& t)
+{
+    if (given != Py_None)
+        t.unsafeGetTensorImpl()->bump_version();
+}
 // the caller's result tensor, checked, or a new one
 at::Tensor result(PyObject* out, at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like)
 {
@@ -164,6 +179,7 @@ at::Tensor result(PyObject* out, at::IntArrayRef sizes, at::ScalarType type, con
         refuse("out is a view that stands for its memory's negative");
     if (t.dim() == 2 ? t.size(1) > 1 && t.stride(1) != 1 : !t.is_contiguous())
         refuse("out must have contiguous rows");
+    writable(t);
     return t;
 }
 int64_t row_stride(const at::Tensor& t)
@@ -242,9 +258,11 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t n)
         q = tensor(args[1], "out");
         packed(q);
         same_device(x, q);
+        writable(q);
     }
     check(cntkq_mx4_quantize_async(handle(x.get_device()), r.data, code, r.rows, r.cols, r.row_stride, r.col_stride, q.data_ptr(), q.numel(),
                                    nullptr, 0));
+    written(args[1], q);
     return Py_BuildValue("(NLL)", THPVariable_Wrap(q), (long long) r.rows, (long long) r.cols);
     END_HANDLE_TH_ERRORS
 }
@@ -260,6 +278,7 @@ PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t n)
     const int code = (int) integer(args[3]);
     const at::Tensor out = result(args[4], {rows, cols}, type_of(code), q);
     check(cntkq_mx4_dequantize_async(handle(q.get_device()), q.data_ptr(), q.numel(), rows, cols, out.data_ptr(), code, row_stride(out)));
+    written(args[4], out);
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }
@@ -280,6 +299,7 @@ PyObject* matmul(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     const at::Tensor out = result(args[7], {m, n}, type_of(code), a);
     check(cntkq_mx4_matmul_async(handle(a.get_device()), a.data_ptr(), a.numel(), m, b.data_ptr(), b.numel(), n, k, bias.data, bias.code,
                                  out.data_ptr(), code, row_stride(out)));
+    written(args[7], out);
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }
@@ -317,6 +337,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     check(cntkq_mx4_linear_async(handle(x.get_device()), r.data, code, r.row_stride, r.rows, w.data_ptr(), w.numel(), n, k, bias.data, bias.code,
                                  y.data_ptr(), out_code, row_stride(y), save ? saved.data_ptr() : nullptr, save ? saved.numel() : 0,
                                  need != 0 ? work.data_ptr() : nullptr, need));
+    written(args[7], y);
     return save ? pair(y, saved) : THPVariable_Wrap(y);
     END_HANDLE_TH_ERRORS
 }
@@ -435,6 +456,9 @@ PyObject* weight_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     check(cntkq_weight_gradient_async(handle(dy.get_device()), r.data, code, r.row_stride, r.rows, r.cols, saved.data_ptr(), saved.numel(), k,
                                       static_cast<float*>(dw.data_ptr()), row_stride(dw), bias ? static_cast<float*>(db.data_ptr()) : nullptr,
                                       accumulate, need != 0 ? work.data_ptr() : nullptr, need));
+    written(args[4], dw);
+    if (bias)
+        written(args[5], db);
     return bias ? pair(dw, db) : THPVariable_Wrap(dw);
     END_HANDLE_TH_ERRORS
 }

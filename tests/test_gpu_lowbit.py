@@ -627,6 +627,59 @@ def test_refusals():
             call()
 
 
+def writes(x, dy, q, kept):
+    """(name, call with an out, a new out) of every function that writes into the caller's tensors."""
+    def new(*sizes):
+        return torch.zeros(*sizes, device="cuda")
+
+    return [("dequantize", lambda out: lowbit.mx4_dequantize(q, torch.float32, out=out), lambda: new(30, 40)),
+            ("matmul", lambda out: lowbit.mx4_matmul(q, q, dtype=torch.float32, out=out), lambda: new(30, 30)),
+            ("linear", lambda out: lowbit.mx4_linear(x, q, out=out), lambda: new(20, 30)),
+            ("linear that keeps x", lambda out: lowbit.mx4_linear(x, q, save=True, out=out), lambda: new(20, 30)),
+            ("dw", lambda out: lowbit.weight_gradient(dy, kept, out=out), lambda: new(30, 40)),
+            ("dw of a pair", lambda out: lowbit.weight_gradient(dy, kept, bias=True, out=(out, None)), lambda: new(30, 40)),
+            ("db of a pair", lambda out: lowbit.weight_gradient(dy, kept, bias=True, out=(None, out)), lambda: new(30))]
+
+
+def test_what_is_written_is_known_to_autograd():
+    x, dy = make(1, 20, 40, torch.float32), make(2, 20, 30, torch.float32)
+    q, kept = lowbit.mx4_quantize(make(3, 30, 40, torch.float32)), lowbit.save8(x)
+    for name, call, new in writes(x, dy, q, kept):
+        out = new()
+        before = out._version
+        call(out)
+        assert out._version == before + 1, name
+        # another operator saved it for its backward pass: that must not go on with other values
+        factor = torch.ones_like(out, requires_grad=True)
+        loss = (factor * out).sum()
+        call(out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        # part of a graph, as a leaf and as a view of one
+        for leaf in (new().requires_grad_(), new().requires_grad_().view(out.shape)):
+            with pytest.raises(QuantizerLogicError):
+                call(leaf)
+            assert not leaf.detach().any(), name
+            with torch.no_grad():
+                call(leaf)
+            assert torch.equal(leaf.detach(), out)
+        with torch.inference_mode():
+            inner = new()
+            call(inner)
+        assert torch.equal(inner, out)
+        with pytest.raises(QuantizerLogicError):
+            call(inner)
+    # a refused call has written nothing, and says nothing else
+    out = torch.zeros(20, 31, device="cuda")
+    with pytest.raises(QuantizerLogicError):
+        lowbit.mx4_linear(x, q, out=out)
+    assert out._version == 0
+    matrix = lowbit.Mx4Matrix(20, 40)
+    before = matrix.buffer._version
+    lowbit.mx4_quantize(x, out=matrix)
+    assert matrix.buffer._version == before + 1
+
+
 def negated(t):
     """A view with t's values over memory that holds their negatives."""
     v = torch._neg_view(-t)
