@@ -13,6 +13,9 @@
 
 #include "../../include/cntk_amd_lowbit.h"
 
+#include <algorithm>
+#include <initializer_list>
+#include <utility>
 #include <vector>
 
 namespace {
@@ -187,6 +190,76 @@ int64_t row_stride(const at::Tensor& t)
     return t.dim() == 2 ? t.stride(0) : (t.dim() == 0 ? 1 : t.size(-1));
 }
 
+struct Bias
+{
+    at::Tensor kept;
+    const void* data = nullptr;
+    int code = CNTKQ_F32;
+};
+
+// The bytes of a matrix in memory: `rows` runs of `length`, `pitch` apart and clear of each other.
+struct Area
+{
+    uintptr_t base;
+    int64_t rows, pitch, length;
+
+    uintptr_t end() const { return base + (rows - 1) * pitch + length; }
+};
+// (of values that lie apart in both directions the closer ones count as one run)
+Area area(const void* data, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride, int64_t size)
+{
+    if (rows > 1 && cols > 1 && col_stride > row_stride)
+    {
+        std::swap(rows, cols);
+        std::swap(row_stride, col_stride);
+    }
+    if (rows == 0 || cols == 0)
+        return {0, 0, 0, 0};
+    Area a = {reinterpret_cast<uintptr_t>(data), rows, row_stride * size, ((cols - 1) * col_stride + 1) * size};
+    if (rows == 1 || a.pitch <= a.length)
+        a = {a.base, 1, 0, (int64_t) (a.end() - a.base)};
+    return a;
+}
+Area area(const at::Tensor& t) // a result, a packed matrix
+{
+    return t.dim() == 2 ? area(t.data_ptr(), t.size(0), t.size(1), t.stride(0), t.size(1) > 1 ? t.stride(1) : 1, t.element_size())
+                        : area(t.data_ptr(), 1, t.numel(), 0, 1, t.element_size());
+}
+Area area(const Rows& r, const at::Tensor& like)
+{
+    return area(r.data, r.rows, r.cols, r.row_stride, r.col_stride, like.element_size());
+}
+Area area(const Bias& b, int64_t n)
+{
+    return b.data == nullptr ? Area{0, 0, 0, 0} : area(b.data, 1, n, 0, 1, b.code == CNTKQ_F32 ? 4 : 2);
+}
+bool overlap(Area a, Area b)
+{
+    if (a.rows == 0 || b.rows == 0 || a.end() <= b.base || b.end() <= a.base)
+        return false;
+    // Runs of one that end before the other's next run are left behind until two meet or none are left. Runs at equal distances either meet
+    // within the first few or never.
+    for (int64_t steps = a.rows > 1 && b.rows > 1 && a.pitch == b.pitch ? 4 : a.rows + b.rows; a.rows > 0 && b.rows > 0 && steps > 0; --steps)
+    {
+        if (b.base < a.base)
+            std::swap(a, b);
+        if (b.base < a.base + a.length)
+            return true;
+        const int64_t behind = a.rows == 1 ? 1 : std::min<int64_t>(a.rows, (b.base - a.base - a.length) / a.pitch + 1);
+        a.base += behind * a.pitch;
+        a.rows -= behind;
+    }
+    return false;
+}
+// The caller's result shares no memory with what the call reads, or with another result of it.
+void apart(const at::Tensor& out, std::initializer_list<Area> others)
+{
+    const Area mine = area(out);
+    for (const Area& a : others)
+        if (overlap(mine, a))
+            refuse("out shares memory with another tensor of the call");
+}
+
 int64_t integer(PyObject* o)
 {
     const long long v = PyLong_AsLongLong(o);
@@ -195,12 +268,6 @@ int64_t integer(PyObject* o)
     return v;
 }
 
-struct Bias
-{
-    at::Tensor kept;
-    const void* data = nullptr;
-    int code = CNTKQ_F32;
-};
 Bias bias_of(PyObject* o, int64_t n, const at::Tensor& like)
 {
     Bias b;
@@ -259,6 +326,7 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t n)
         packed(q);
         same_device(x, q);
         writable(q);
+        apart(q, {area(r, x)});
     }
     check(cntkq_mx4_quantize_async(handle(x.get_device()), r.data, code, r.rows, r.cols, r.row_stride, r.col_stride, q.data_ptr(), q.numel(),
                                    nullptr, 0));
@@ -277,6 +345,8 @@ PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t n)
     const int64_t rows = integer(args[1]), cols = integer(args[2]);
     const int code = (int) integer(args[3]);
     const at::Tensor out = result(args[4], {rows, cols}, type_of(code), q);
+    if (args[4] != Py_None)
+        apart(out, {area(q)});
     check(cntkq_mx4_dequantize_async(handle(q.get_device()), q.data_ptr(), q.numel(), rows, cols, out.data_ptr(), code, row_stride(out)));
     written(args[4], out);
     return THPVariable_Wrap(out);
@@ -297,6 +367,8 @@ PyObject* matmul(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     const Bias bias = bias_of(args[5], n, a);
     const int code = (int) integer(args[6]);
     const at::Tensor out = result(args[7], {m, n}, type_of(code), a);
+    if (args[7] != Py_None)
+        apart(out, {area(a), area(b), area(bias, n)});
     check(cntkq_mx4_matmul_async(handle(a.get_device()), a.data_ptr(), a.numel(), m, b.data_ptr(), b.numel(), n, k, bias.data, bias.code,
                                  out.data_ptr(), code, row_stride(out)));
     written(args[7], out);
@@ -328,6 +400,8 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     c10::SmallVector<int64_t, 6> sizes(x.sizes().begin(), x.sizes().end());
     sizes.back() = n;
     const at::Tensor y = result(args[7], sizes, type_of(out_code), x);
+    if (args[7] != Py_None)
+        apart(y, {area(r, x), area(w), area(bias, n)});
     at::Tensor saved, work;
     if (save)
         saved = bytes(cntkq_save8_bytes(r.rows, k), x);
@@ -447,9 +521,15 @@ PyObject* weight_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         refuse("accumulate needs every result's tensor to add to");
     const Rows r = rows_of(dy, true);
     const at::Tensor dw = result(args[4], {r.cols, k}, at::kFloat, dy);
+    if (args[4] != Py_None)
+        apart(dw, {area(r, dy), area(saved)});
     at::Tensor db, work;
     if (bias)
+    {
         db = result(args[5], {r.cols}, at::kFloat, dy);
+        if (args[5] != Py_None)
+            apart(db, {area(r, dy), area(saved), area(dw)});
+    }
     const size_t need = cntkq_weight_gradient_workspace_bytes(r.rows, r.cols, k, code);
     if (need != 0)
         work = bytes(need, dy);

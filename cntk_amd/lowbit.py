@@ -15,7 +15,7 @@ the backward pass in 8 bits, and the weight gradient read from what was kept -- 
 Element types: float32, float16, bfloat16. Tensors of more than two dimensions are taken as rows of their last one. Everything is issued
 on torch's current stream of the tensors' device; nothing waits and nothing is kept between calls. As with any torch operator, a tensor made on
 another stream needs that stream's work to be over or waited for. The functions take part in no autograd graph; the modules do. An `out` that
-requires grad is refused while gradients are recorded, and what is written raises its version, so that a backward pass that needs the old values says so.
+requires grad is refused while gradients are recorded, and so is one that shares memory with another tensor of the call; what is written raises its version, so that a backward pass that needs the old values says so.
 Errors are this package's: QuantizerLogicError for arguments that do not fit, QuantizerError for a failed device call.
 """
 import ctypes

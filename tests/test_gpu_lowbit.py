@@ -680,6 +680,53 @@ def test_what_is_written_is_known_to_autograd():
     assert matrix.buffer._version == before + 1
 
 
+def test_results_share_no_memory_with_the_rest_of_a_call():
+    square = lowbit.mx4_quantize(make(1, 40, 40, torch.float32))
+    x = make(2, 40, 40, torch.float32)
+    kept = lowbit.save8(x)
+    store = torch.zeros(1 << 16, device="cuda")
+
+    def at(offset, rows, cols, stride):
+        return store.as_strided((rows, cols), (stride, 1), offset)
+
+    refused = [
+        lambda: lowbit.mx4_linear(x, square, out=x),
+        lambda: lowbit.mx4_linear(at(0, 40, 40, 40), square, out=at(1599, 40, 40, 40)),
+        lambda: lowbit.mx4_linear(at(1600, 40, 40, 40), square, out=at(1, 40, 40, 40)),
+        lambda: lowbit.mx4_linear(at(0, 40, 40, 100), square, out=at(39, 40, 40, 100)),  # one column
+        lambda: lowbit.mx4_linear(at(0, 40, 40, 100), square, out=at(61, 40, 40, 100)),  # the next row's first one
+        lambda: lowbit.mx4_linear(at(0, 40, 40, 100), square, out=at(40, 40, 40, 120)),  # rows that come nearer
+        lambda: lowbit.mx4_linear(at(0, 1, 40, 40).expand(40, 40), square, out=at(0, 40, 40, 40)),
+        lambda: lowbit.mx4_linear(x, square, at(0, 1, 40, 40)[0], out=at(0, 40, 40, 40)),
+        lambda: lowbit.mx4_linear(x, lowbit.Mx4Matrix(40, 40, store.view(torch.uint8)[:square.buffer.numel()]), out=at(0, 40, 40, 40)),
+        lambda: lowbit.mx4_matmul(square, lowbit.Mx4Matrix(40, 40, store.view(torch.uint8)[:square.buffer.numel()]), dtype=torch.float32, out=at(0, 40, 40, 40)),
+        lambda: lowbit.mx4_matmul(square, square, at(0, 1, 40, 40)[0], dtype=torch.float32, out=at(0, 40, 40, 40)),
+        lambda: lowbit.mx4_dequantize(lowbit.Mx4Matrix(40, 40, store.view(torch.uint8)[:square.buffer.numel()]), torch.float32, out=at(9, 40, 40, 40)),
+        lambda: lowbit.mx4_quantize(at(0, 40, 40, 40), out=lowbit.Mx4Matrix(40, 40, store.view(torch.uint8)[:square.buffer.numel()])),
+        lambda: lowbit.mx4_quantize(at(0, 40, 40, 40).t(), out=lowbit.Mx4Matrix(40, 40, store.view(torch.uint8)[:square.buffer.numel()])),
+        lambda: lowbit.weight_gradient(at(0, 40, 40, 40), kept, out=at(40, 40, 40, 40)),
+        lambda: lowbit.weight_gradient(at(0, 40, 40, 40), kept, bias=True, out=(None, store[1599:1639])),
+        lambda: lowbit.weight_gradient(x, kept, bias=True, out=(at(0, 40, 40, 40), store[1599:1639])),
+        lambda: lowbit.weight_gradient(x, lowbit.Saved8(x.shape, x.dtype, store.view(torch.uint8)[:kept.buffer.numel()]), out=at(0, 40, 40, 40)),
+    ]
+    for i, call in enumerate(refused):
+        with pytest.raises(QuantizerLogicError, match="shares memory"):
+            call()
+        assert not store.any(), i
+    # side by side: rows of one between the rows of the other, at equal distances and at others, and end to end
+    want = lowbit.mx4_linear(x, square)
+    for (x_at, x_stride), (out_at, out_stride) in [((0, 80), (40, 80)), ((40, 80), (0, 80)), ((0, 80), (1000 * 40, 80)), ((0, 40), (1600, 40)), ((1600, 40), (0, 40)),
+                                                   ((40, 160), (0, 80)), ((0, 80), (40, 160)), ((3, 91), (45, 91)), ((91, 91), (43, 91)), ((0, 1640), (40, 40))]:
+        store.fill_(float("nan"))
+        v, out = at(x_at, 40, 40, x_stride), at(out_at, 40, 40, out_stride)
+        v.copy_(x)
+        lowbit.mx4_linear(v, square, out=out)
+        assert torch.equal(out, want) and torch.equal(v, x)
+    store.zero_()
+    dw, db = lowbit.weight_gradient(x, kept, bias=True, out=(at(0, 40, 40, 41), store[1639:1679]))
+    assert torch.equal(dw, lowbit.weight_gradient(x, kept)) and torch.equal(db, lowbit.weight_gradient(x, kept, bias=True)[1])
+
+
 def negated(t):
     """A view with t's values over memory that holds their negatives."""
     v = torch._neg_view(-t)
