@@ -371,6 +371,33 @@ def test_activation_gradient_against_differences(kind):
     assert (np.abs(slope - d) <= allowed)[:, :31][smooth[:, :31]].all()
 
 
+def test_exponentials_keep_their_places():
+    """Sigmoid and SiLU far below zero in single precision, where an absolute bound asks for nothing. e^-x: its last place (2^-23) and half a place where the
+    remainder is multiplied on; half a place each for the sum and the quotient: 2^-21.6 of the result. The slopes take that factor and one that is
+    within 2^-21.7 of itself (sigmoid: 1 - f of f up to a half; SiLU: 1 + x (1 - f), whose terms cancel by a third at most below -3) and round their
+    product: 2^-20.5. Each bound is taken at the next power of two."""
+    x = -torch.linspace(3.0, 85.0, 32 * 4096, device="cuda").view(4096, 32)
+    a = np64(x)
+    for kind in ("sigmoid", "silu"):
+        y, kept = lowbit.activation_forward(kind, x)
+        f, _ = ref.activation(kind, a)
+        assert (np.abs(np64(y) - f) <= 2.0 ** -21 * np.abs(f)).all()
+        _, d = ref.activation(kind, np64(kept.values()))
+        got = np64(lowbit.activation_backward(torch.ones_like(x), kept))
+        assert (np.abs(got - d) <= 2.0 ** -20 * np.abs(d)).all()
+        # gated, the function is a factor
+        y, kept = lowbit.activation_forward(kind, torch.ones_like(x), x)
+        assert (np.abs(np64(y) - f) <= 2.0 ** -21 * np.abs(f)).all()
+    # where it is 0 or infinite
+    far = torch.tensor([[-1e30, -3.4e38, -200.0, -89.0, 89.0, 200.0, 1e30, 3.4e38, float("inf"), float("-inf"), float("nan")]], device="cuda")
+    y, _ = lowbit.activation_forward("sigmoid", far)
+    assert torch.equal(y[0, 4:9], torch.ones(5, device="cuda")) and float(y[0, :4].abs().max()) < 1e-37 and y[0, 9] == 0.0 and torch.isnan(y[0, 10])
+    y, _ = lowbit.activation_forward("silu", far)
+    assert torch.equal(y[0, 4:9], far[0, 4:9]) and float(y[0, :4].abs().max()) < 1e-35
+    _, kept = lowbit.activation_forward("sigmoid", far[:, :8].repeat_interleave(32, 1))
+    assert float(lowbit.activation_backward(torch.ones(1, 256, device="cuda"), kept).abs().max()) < 1e-37
+
+
 # ---- weight gradients -----------------------------------------------------------------------------
 
 
