@@ -532,6 +532,44 @@ def test_a_weight_gradient_of_more_rows_than_one_pair_of_launches_takes():
         assert ((db.double() - a.sum(0)).abs() <= 4 * 2.0 ** -23 * m ** 0.5 * a.abs().sum(0).max()).all()
 
 
+def whole_numbers(seed, rows, cols, most, dtype):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(-most, most + 1, (rows, cols), generator=g, device="cuda", dtype=torch.int8).to(dtype)
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.bfloat16, 520), (torch.bfloat16, 521), (torch.float16, 520)], ids=["bf16 as it lies", "bf16 turned", "f16 turned"])
+def test_a_weight_gradient_in_several_pairs_of_launches(dtype, n):
+    """Many results of more than 2^21 rows: the second piece's rows, codes and scales, added to the first one's results. Whole numbers, so small that every
+    product and sum in 32 bits is exact, whatever the order."""
+    m, k = (1 << 21) + 77, 2024
+    x, dy = whole_numbers(1, m, k, 3, torch.bfloat16), whole_numbers(2, m, n, 2, dtype)
+    x[:, ::32] *= torch.where(torch.arange(m, device="cuda") % 3 == 0, 20.0, 1.0).to(torch.bfloat16)[:, None]  # scales that differ from row to row
+    kept = lowbit.save8(x)
+    want, sums = torch.zeros(n, k, device="cuda"), torch.zeros(n, device="cuda")
+    for row in range(0, m, 1 << 18):
+        a, b = dy[row:row + (1 << 18)].float(), x[row:row + (1 << 18)].float()
+        want += a.t().contiguous() @ b
+        sums += a.sum(0)
+    assert float(want.abs().max()) < 2 ** 23
+    dw, db = lowbit.weight_gradient(dy, kept, bias=True)
+    assert torch.equal(dw, want) and torch.equal(db, sums)
+    lowbit.weight_gradient(dy, kept, bias=True, out=(dw, db), accumulate=True)
+    assert torch.equal(dw, 2.0 * want) and torch.equal(db, 2.0 * sums)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n", [24, 23])
+def test_column_sums_in_several_pairs_of_launches(n, dtype):
+    m = (1 << 22) + 1
+    dy = whole_numbers(3, m, n, 2, dtype)
+    sums = dy.double().sum(0).float()
+    kept = lowbit.save8(torch.zeros(m, 0, dtype=dtype, device="cuda"))
+    dw, db = lowbit.weight_gradient(dy, kept, bias=True)
+    assert dw.shape == (n, 0) and torch.equal(db, sums)
+    lowbit.weight_gradient(dy, kept, bias=True, out=(dw, db), accumulate=True)
+    assert torch.equal(db, 2.0 * sums)
+
+
 def test_weight_gradients_of_what_is_not_finite():
     """An infinity or a NaN of dy reaches its own row of dw; one of x its block's columns."""
     for dtype in DTYPES:
