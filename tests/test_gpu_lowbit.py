@@ -371,6 +371,44 @@ def test_activation_gradient_against_differences(kind):
     assert (np.abs(slope - d) <= allowed)[:, :31][smooth[:, :31]].all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,cols", [(5, 8), (131, 40), (67, 2048), (3, 4104)])
+def test_activations_of_whole_eights(rows, cols, kind, dtype):
+    """Widths that are a multiple of eight take kernels of their own: a ragged last block, a row on all lanes of a workgroup, one on several; rows
+    that leave a workgroup partly empty. Inputs as they lie and as columns of a wider matrix, at any element."""
+    x, gate, dy = make(rows, rows, cols, dtype, 0.7), make(rows + 1, rows, cols, dtype, 0.7), make(rows + 2, rows, cols, dtype, 0.3)
+    x64, g64, dy64 = np64(x), np64(gate), np64(dy)
+    x8, g8 = ref.save8(x64)[2], ref.save8(g64)[2]
+    smooth = 2.0 ** -19 * (kind != "relu")
+
+    def inside(t):
+        wide = torch.full((rows, cols + 5), float("nan"), dtype=dtype, device="cuda")
+        wide[:, 3:3 + cols] = t
+        return wide[:, 3:3 + cols]
+
+    f, _ = ref.activation(kind, x64)
+    _, d = ref.activation(kind, x8)
+    for given, back in ((x, dy), (inside(x), inside(dy))):
+        y, kept = lowbit.activation_forward(kind, given)
+        check_save8(kept, x)
+        close(y, f, smooth * (1 + np.abs(x64)), dtype)
+        close(lowbit.activation_backward(back, kept), dy64 * d, np.abs(dy64) * smooth * (1 + np.abs(x8)), dtype)
+    f, _ = ref.activation(kind, g64)
+    f8, d8 = ref.activation(kind, g8)
+    for given, by, back in ((x, gate, dy), (inside(x), inside(gate), inside(dy))):
+        y, kept = lowbit.activation_forward(kind, given, by)
+        check_save8(kept, x)
+        codes, scales = ref.unpack_save8(kept.gate.cpu().numpy(), rows, cols)
+        np.testing.assert_array_equal(codes, ref.save8(g64)[0])
+        np.testing.assert_array_equal(scales, ref.save8(g64)[1])
+        close(y, f * x64, np.abs(x64) * 2.0 ** -19 * (1 + np.abs(g64)), dtype)
+        dx, dgate = lowbit.activation_backward(back, kept)
+        near = 2.0 ** -19 * (1 + np.abs(g8))
+        close(dx, dy64 * f8, np.abs(dy64) * near, dtype)
+        close(dgate, dy64 * x8 * d8, np.abs(dy64 * x8) * near, dtype)
+
+
 def test_exponentials_keep_their_places():
     """Sigmoid and SiLU far below zero in single precision, where an absolute bound asks for nothing. e^-x: its last place (2^-23) and half a place where the
     remainder is multiplied on; half a place each for the sum and the quotient: 2^-21.6 of the result. The slopes take that factor and one that is
