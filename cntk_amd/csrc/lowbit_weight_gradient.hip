@@ -1,6 +1,7 @@
 // The weight gradient of a linear layer whose input was kept in 8 bits: dw[n, k] = sum over m of dy[m, n] x8[m, k], and the
 // column sums of dy. x8's values are bfloat16 numbers as they are; dy of a wider type is a sum of bfloat16 numbers (half precision: two,
-// single: three), each multiplied in turn, so every product is exact and the sums are in 32 bits.
+// single: three), each multiplied in turn, so every product is exact and the sums are in 32 bits. (bfloat16 ends at 2^-133: what a single-precision dy has below
+// that, of numbers under 2^-110, is not multiplied. Half precision's numbers are nowhere near.)
 //
 // Both factors run along memory in the axis that is not summed over, and the matrix unit wants the other. For many results a first launch turns
 // them over into tiles in the workspace (dy: 2 bytes an element and term, x8: 2), reading each once; the second multiplies tiles. Turning
@@ -147,7 +148,7 @@ __device__ __forceinline__ u32x4 eight_upper_halves(float a, float b, float c, f
     return u32x4{upper_halves(a, b), upper_halves(c, d), upper_halves(e, f), upper_halves(g, h)};
 }
 
-// What the upper halves leave, exactly; FIRST: and nothing of an infinity or a NaN.
+// What the upper halves leave, exactly down to 2^-133; FIRST: and nothing of an infinity or a NaN.
 template <bool FIRST>
 __device__ __forceinline__ void take_upper_halves(float (&v)[8][2])
 {

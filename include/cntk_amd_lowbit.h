@@ -92,7 +92,8 @@ int cntkq_activation_backward_async(cntkq_quantizer* h, int kind, const void* dy
                                     int64_t dgate_stride);
 
 /* dw[j, c] = sum over i of dy[i, j] x8[i, c] (dy m x n, rows contiguous; x8 m x k as kept; dw n x k in 32 bits) and, unless
- * db is null, db[j] = sum over i of dy[i, j]. Products exact, sums in 32 bits, in an order that depends on the sizes alone.
+ * db is null, db[j] = sum over i of dy[i, j]. Products exact (of a single-precision dy below 2^-110 up to 2^-133 is left out of dw), sums in 32 bits, in an
+ * order that depends on the sizes alone.
  * accumulate: added to what dw and db hold. The workspace (16-byte aligned) is free again once the call's work on the stream is done. */
 size_t cntkq_weight_gradient_workspace_bytes(size_t m, size_t n, size_t k, int dtype);
 int cntkq_weight_gradient_async(cntkq_quantizer* h, const void* dy, int dtype, int64_t dy_stride, size_t m, size_t n, const void* saved,

@@ -608,6 +608,32 @@ def test_column_sums_in_several_pairs_of_launches(n, dtype):
     assert torch.equal(db, 2.0 * sums)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,k,n", [(40, 64, 50), (1100, 40, 30), (40, 1500, 1501)])
+def test_weight_gradients_of_the_smallest_values(m, k, n, dtype):
+    """Gradients and kept inputs down to the smallest number of the type, subnormal ones among them, against large factors. Of a single-precision gradient the
+    bits below 2^-133 are not multiplied; everything else is."""
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+    low, high = (-24, 10) if dtype == torch.float16 else (-149, -99)
+    dy = torch.randn(m, n, generator=g, device="cuda") * torch.exp2(torch.randint(low, high, (m, n), generator=g, device="cuda").float())
+    dy = dy.to(dtype)
+    assert torch.isfinite(dy).all()
+    kept = lowbit.save8(torch.randn(m, k, generator=g, device="cuda") * 2.0 ** 30)
+    a, b = dy.double(), kept.values(torch.float32).double()
+    want, sizes = a.t() @ b, a.abs().t() @ b.abs()
+    left_out = 2.0 ** -133 * b.abs().sum(0) if dtype == torch.float32 else 0.0
+    got = lowbit.weight_gradient(dy, kept)
+    assert ((got.double() - want).abs() <= (3 * m + 1) * 2.0 ** -23 * sizes + left_out + (3 * m + 1) * 2.0 ** -149).all()
+    # the smallest kept inputs
+    x = torch.randn(m, k, generator=g, device="cuda") * torch.exp2(torch.randint(-149, -100, (m, k // 2), generator=g, device="cuda").float()).repeat(1, 2)
+    kept = lowbit.save8(x)
+    dy = (torch.randn(m, n, generator=g, device="cuda") * 2.0 ** 14).to(dtype).clamp(-60000.0, 60000.0)
+    a, b = dy.double(), kept.values(torch.float32).double()
+    want, sizes = a.t() @ b, a.abs().t() @ b.abs()
+    assert float(want.abs().max()) > 0.0
+    assert ((lowbit.weight_gradient(dy, kept).double() - want).abs() <= (3 * m + 1) * 2.0 ** -23 * sizes + (3 * m + 1) * 2.0 ** -149).all()
+
+
 def test_weight_gradients_of_what_is_not_finite():
     """An infinity or a NaN of dy reaches its own row of dw; one of x its block's columns."""
     for dtype in DTYPES:
