@@ -524,6 +524,8 @@ uint32_t run_tiles(size_t m_tiles, size_t n, size_t k)
 }
 Workspace workspace_of(size_t m, size_t n, size_t k, int dtype)
 {
+    if (n == 0) // nothing to make, and no workgroups to deal the depth to
+        return {0, 0, 0};
     if (way_of(m, n, k, dtype) == Way::kDirect)
         return {0, 0, 0};
     if (way_of(m, n, k, dtype) == Way::kParts)

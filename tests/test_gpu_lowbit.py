@@ -545,6 +545,23 @@ def test_column_sums_of_a_layer_without_inputs(m, n, dtype):
     assert ((db.double() - a.sum(0)).abs() <= (m + 1) * 2.0 ** -23 * a.abs().sum(0)).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m", [0, 1, 40, 1024, 1025, 5000])
+def test_layers_without_results(m, dtype):
+    """No columns of the gradient, of any number of rows; then no rows."""
+    x = make(1, max(m, 1), 40, dtype)[:m]
+    w = lowbit.mx4_quantize(torch.zeros(0, 40, dtype=dtype, device="cuda"))
+    y, kept = lowbit.mx4_linear(x, w, save=True)
+    assert y.shape == (m, 0) and lowbit.mx4_linear(x, w).shape == (m, 0)
+    assert torch.equal(kept.buffer, lowbit.save8(x).buffer)
+    dw, db = lowbit.weight_gradient(torch.zeros(m, 0, dtype=dtype, device="cuda"), kept, bias=True)
+    assert dw.shape == (0, 40) and db.shape == (0,)
+    assert lowbit.weight_gradient(torch.zeros(m, 0, dtype=dtype, device="cuda"), kept, out=dw, accumulate=True) is dw
+    # the input gradient: a product without an inner side
+    dx = lowbit.mx4_linear(torch.zeros(m, 0, dtype=dtype, device="cuda"), lowbit.mx4_quantize(torch.zeros(40, 0, dtype=dtype, device="cuda")))
+    assert dx.shape == (m, 40) and not dx.any()
+
+
 def test_a_large_weight_gradient():
     m, k, n = 70, 4100, 4200
     x, dy = make(1, m, k, torch.bfloat16), make(2, m, n, torch.bfloat16)

@@ -26,6 +26,23 @@ def test_packed_sizes():
     assert L.cntkq_weight_gradient_workspace_bytes(5, 6, 7, 9) == 0
 
 
+def test_sizes_of_what_is_empty():
+    """Any side may be 0, alone or with others: no result is no workspace, whatever the number of rows."""
+    L = lowbit._bind()
+    sides = (0, 1, 16, 17, 1024, 1025, 2000, 1 << 22)
+    for m in sides:
+        for k in sides:
+            for dtype in (0, 1, 2):
+                assert L.cntkq_weight_gradient_workspace_bytes(m, 0, k, dtype) == 0
+                L.cntkq_weight_gradient_workspace_bytes(m, k, 0, dtype)
+                L.cntkq_weight_gradient_workspace_bytes(0, m, k, dtype)
+                for save in (0, 1):
+                    assert L.cntkq_mx4_linear_workspace_bytes(0, m, k, dtype, save) == 0
+                    assert L.cntkq_mx4_linear_workspace_bytes(m, k, 0, dtype, save) == 0
+                    L.cntkq_mx4_linear_workspace_bytes(m, 0, k, dtype, save)
+            assert L.cntkq_mx4_bytes(m, 0) == L.cntkq_mx4_bytes(0, k) == L.cntkq_save8_bytes(m, 0) == L.cntkq_save8_bytes(0, k) == 0
+
+
 def test_refusals_before_the_device():
     L = lowbit._bind()
     h = ctypes.create_string_buffer(4096)  # never read: the arguments are refused first
