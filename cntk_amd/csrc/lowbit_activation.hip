@@ -142,7 +142,7 @@ __device__ __forceinline__ void fetch(const RowGrid& g, const Place& p, const vo
 }
 
 // y = f(x), or f(gate) x; x (and the gate) kept in 8 bits. Bound by memory: each value read once, written once, 33/32 bytes kept.
-// Gated, 8192 x 4096 in bfloat16: 271 MB in 52 us, 5.2 TB/s, a large copy's rate; 1024 x 2048 in single precision 5.7 to 6.1 us.
+// Gated, 8192 x 4096 in bfloat16: 271 MB in 52 us, 5.2 TB/s, a large copy's rate; 1024 x 2048 in single precision 6.1 us.
 template <int KIND, int DT, bool GATED, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void activation_forward_kernel(ActivationForward a, RowGrid g)
 {
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(kThreads) void activation_forward_kernel(Activation
 }
 
 // dx = dy f'(x8); gated dx = dy f(g8), dgate = dy x8 f'(g8). Bound by memory: 270 MB in 48 us,
-// and 5.6 to 5.9 us, for the matrices above.
+// and 6.0 us, for the matrices above.
 template <int KIND, int DT, bool GATED, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void activation_backward_kernel(ActivationBackward a, RowGrid g)
 {

@@ -164,7 +164,7 @@ __device__ __forceinline__ void take_upper_halves(float (&v)[8][2])
 
 // Wavefront w of a workgroup has eight rows of a tile's 32; a lane has four columns of x8 or two of dy, and writes for each the
 // eight values that one lane of the matrix instruction takes. The next tile's loads are on their way while one is turned over. Bound by memory:
-// 4096 rows of 9304 and 2048 columns in bfloat16, 202 MB, 42 us.
+// 4096 rows of 9304 and 2048 columns in half precision, 254 MB, 66 to 69 us, in single precision, 407 MB, 89 to 91; of 9303 in bfloat16, value by value, 54.
 __device__ __forceinline__ void turn_x(const Pack& a, uint32_t chunk, uint32_t first, uint32_t last)
 {
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = chunk * kXCols + lane * 4;
@@ -468,7 +468,8 @@ __global__ __launch_bounds__(512) void weight_gradient_direct_kernel(Pack a, Out
 // 16384 x 1024 x 512 77 / 83, but 2048 x 2048 x 1024 34 / 27. Narrow, in bfloat16: 4096 x 65536 x 64 189 / 198, 4096 x 64 x 65536 211 / 403,
 // 300 x 1000000 x 40 238 / 296 (single precision 317 / 1402), but 4096 x 65536 x 128 345 / 212. In parts and with tiles, in single precision:
 // 1500 x 128 x 128 9.0 / 10.4, 6886 x 1024 x 128 19 / 43, 65536 x 128 x 128 33 / 185, 1000000 x 64 x 64 418 / 4184; in bfloat16 1500 x 128 x 128 7.7 / 7.6,
-// 4096 x 512 x 512 17 / 24, 65536 x 512 x 512 152 / 155, 1000000 x 64 x 64 304 / 2043.
+// 4096 x 512 x 512 17 / 24, 65536 x 512 x 512 152 / 155, 1000000 x 64 x 64 304 / 2043. Just above 2^18 results nothing cuts the depth, and a deep one has
+// few workgroups for it; in one launch and with tiles: 16384 x 520 x 512 in bfloat16 86 / 127, in single precision 103 / 352, 65536 x 520 x 512 316 / 474 and 426 / 1872.
 enum class Way
 {
     kDirect,
@@ -553,7 +554,8 @@ hipError_t multiply(hipStream_t s, const Tiles& x, const DY& y, uint32_t depth, 
 
 // Blocks of 160 x 256, 128 x 256, 128 x 128 or 64 x 128 (rows of dw first): as for the 4-bit products, and with two heights of the large ones, of
 // which one may need a round less. Stage times from products of 8192^3 (1050, 970, 1068 and 1429 us); m x n x k, us in the same order:
-// 4096 x 9304 x 2048 146 / 184 / 158 / 223 (dy in tiles; as it lies 147), 2048^3 51 / 45 / 25.1 / 27.5, 257 x 2048 x 429 12.5 / 10.1 / 7.6 / 6.3.
+// 4096 x 9304 x 2048 146 / 184 / 158 / 223 (dy in tiles; as it lies 147; of 160 x 256 the kernel keeps 15 to 18 registers too many, 64 to 76 bytes a lane,
+// which go through memory at the change of blocks but not in the stages between), 2048^3 51 / 45 / 25.1 / 27.5, 257 x 2048 x 429 12.5 / 10.1 / 7.6 / 6.3.
 template <bool ACCUMULATE, typename DY>
 hipError_t multiply_best(hipStream_t s, const Tiles& x, const DY& y, uint32_t depth, const Output& o, const Sums& b)
 {
